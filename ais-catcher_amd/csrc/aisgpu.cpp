@@ -1373,8 +1373,9 @@ int aisgpu_create(const aisgpu_cfg* cfg, aisgpu_t** out) {
 		// pipeline; sharing a SIMD with throughput kernels more than doubles its run time (every foreign VALU
 		// instruction delays its next dependent one).  It therefore gets CUs of its own: CU-mask bits 0..7 are one
 		// CU in each of the 8 XCDs (tools/microbench_cumask.hip), 3% of the chip; the back-end streams use the rest.
-		// The front stream is a plain stream of the LOWEST queue priority: the workgroup dispatcher then prefers the back end's
-		// workgroups whenever a slot frees up (2-3 % per step, profiles/r02_expI.txt .. r02_expK.txt).
+		// The front stream is a plain stream over all CUs.  Non-blocking: a stream with a CU mask waits for the caller's work on
+		// the legacy default stream.  Every stream has the default queue priority: work on streams of different priorities can
+		// stop for good on this hardware.
 		int n_cu = 0;
 		HIPCHK(hipDeviceGetAttribute(&n_cu, hipDeviceAttributeMultiprocessorCount, cfg->device_id));
 #ifndef AISGPU_RESERVE_CUS
@@ -1394,10 +1395,8 @@ int aisgpu_create(const aisgpu_cfg* cfg, aisgpu_t** out) {
 			const int words = (n_cu + 31) / 32;
 			std::vector<uint32_t> lat(words, 0u), rest(words, 0u);
 			for (int i = 0; i < n_cu; i++) (i < reserve ? lat : rest)[i / 32] |= 1u << (i % 32);
-			int least = 0, greatest = 0;
-			const bool prio = hipDeviceGetStreamPriorityRange(&least, &greatest) == hipSuccess && least != greatest; // (the front stream at the lowest queue priority: the dispatcher prefers the back end's workgroups whenever a slot frees up)
 			// (a runtime without CU masks falls back to ordinary streams: same results, the recurrence just shares its SIMDs)
-						masked = (prio ? hipStreamCreateWithPriority(&h->stream, hipStreamNonBlocking, least) : hipExtStreamCreateWithCUMask(&h->stream, (uint32_t)words, rest.data())) == hipSuccess;
+			masked = hipStreamCreateWithFlags(&h->stream, hipStreamNonBlocking) == hipSuccess;
 			masked = masked && hipExtStreamCreateWithCUMask(&h->s1, (uint32_t)words, rest.data()) == hipSuccess;
 			masked = masked && hipExtStreamCreateWithCUMask(&h->s3, (uint32_t)words, lat.data()) == hipSuccess;
 			masked = masked && hipExtStreamCreateWithCUMask(&h->s4, (uint32_t)words, rest.data()) == hipSuccess;

@@ -23,3 +23,11 @@ def test_no_writes_through_the_scalar_data_cache():
     scalar_write = re.compile(r"\bs_((buffer_|scratch_)?(store|atomic)|dcache_(wb|discard))", re.I)
     for name, text in _hip_sources():
         assert not scalar_write.search(text), name
+
+
+def test_streams_have_the_default_priority():
+    """Work on streams of different queue priorities can stop for good on this hardware: no source asks for one."""
+    sources = _texts("ais-catcher_amd/*.py", "ais-catcher_amd/host/*.cpp", "ais-catcher_amd/host/*.h", "integration/reference/Source/DSP/GPU/*",
+                     "tools/*.py", "bench.py")
+    for name, text in _hip_sources() + sources:
+        assert not re.search(r"StreamCreateWithPriority|StreamPriorityRange|\bpriority\s*=|is_high_priority_stream", text), name
