@@ -102,8 +102,8 @@ __device__ __forceinline__ float2 cic5_small(const float4* lvl4, int t) {
 // there is no LDS traffic and no synchronisation at all; only the two channel filters behind the rotator use a
 // small wave-private LDS ring.  Arithmetic and pairing are identical to the LDS variant (cic5_dec_chunk).
 // ------------------------------------------------------------------------------------------
-// complex samples as native 2-vectors: an add is one v_pk_add_f32 on an aligned register pair and (re, im) stay
-// together (with the float2 struct the SLP vectoriser re-pairs components of different samples and pays for it in moves)
+// complex samples as native 2-vectors: (re, im) stay together.  The build turns packed f32 instructions off (Makefile), so an
+// operation on a pair is two plain ones.
 
 __device__ __forceinline__ float dpp_wave_shr1(float old_lane0, float src) { // lane l <- src[l-1]; lane 0 keeps old_lane0
 	return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old_lane0), __float_as_int(src), 0x138, 0xF, 0xF, false));
@@ -1969,11 +1969,7 @@ __global__ __launch_bounds__(64) void k2_cgf_refine(K2Params p) {
 // The groups of window w are those whose LAST sample lies in it.  Workgroup ids put a channel's windows on one XCD, one behind the
 // other (the rows' lines that two windows share meet in that L2).
 // ------------------------------------------------------------------------------------------
-__device__ __forceinline__ c2 pk_sub_add(c2 a, c2 b) { // (a.x - b.x, a.y + b.y) in one packed add (x - y == x + (-y) exactly)
-	c2 r;
-	asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-	return r;
-}
+__device__ __forceinline__ c2 sub_add(c2 a, c2 b) { return c2{ a.x - b.x, a.y + b.y }; } // the sums of a complex product
 
 constexpr int K6_HL = 5;                    // segments of the previous window derotated again as the window's halo
 constexpr int K6_HALO = K6_HL * CK_SEG - 1; // = 44 samples: segments 52..56 (the FIR needs 20; the FM branch 37: 36 of the Receiver filter + Demod::FM's prev)
@@ -2013,7 +2009,7 @@ __device__ __forceinline__ void k6_window_body(const K6Params& p, int chain, int
 #pragma unroll
 			for (int m = 0; m < CK_SEG; m++) {
 				rot = rot.xx * st + rot.yy * st_sw;                       // rot *= rot_step
-				const c2 v = pk_sub_add(rot * d[m].x, rot.yx * d[m].y);   // data * rot = (d.x r.x - d.y r.y, d.x r.y + d.y r.x)
+				const c2 v = sub_add(rot * d[m].x, rot.yx * d[m].y);   // data * rot = (d.x r.x - d.y r.y, d.x r.y + d.y r.x)
 				if (m < CK_SEG - 1 || si < CK_USED - 1) y[m] = make_float2(v.x, v.y);
 			}
 		}
@@ -2999,7 +2995,7 @@ __device__ __forceinline__ void k46_body(const K46Params& q, int trip, int chunk
 #pragma unroll
 			for (int m = 0; m < CK_SEG; m++) {
 				rot = rot.xx * st + rot.yy * st_sw;                       // rot *= rot_step
-				const c2 v = pk_sub_add(rot * d[m].x, rot.yx * d[m].y);   // data * rot
+				const c2 v = sub_add(rot * d[m].x, rot.yx * d[m].y);   // data * rot
 				if (m < CK_SEG - 1 || si < CK_USED - 1) y[m] = make_float2(v.x, v.y);
 			}
 		}

@@ -1,6 +1,6 @@
 // tools/microbench_anyorder.hip -- does hipExtAnyOrderLaunch let the next kernel of a stream begin while the previous one drains?
 // (hip_ext.h says the flag is "not supported on AMD GFX9xx boards" for the module launch; this measures what gfx950 does.)
-//   hipcc --offload-arch=gfx950 -O3 tools/microbench_anyorder.hip -o /tmp/mb_anyorder && /tmp/mb_anyorder
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_anyorder.hip -o /tmp/mb_anyorder && /tmp/mb_anyorder
 // Test 1: two launches of a kernel whose workgroup 0 runs 2 ms and all others 10 us.  In order: 4 ms; overlapped: ~2 ms.
 // Test 2: the front end's shape -- 6,144 one-wave workgroups of ~100 us +- 20 % on 3,072 slots (LDS-capped), 20 launches back to back.
 #include <hip/hip_runtime.h>

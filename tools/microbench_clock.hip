@@ -1,5 +1,6 @@
 // tools/microbench_clock.hip -- what does s_memtime count, and how fast does a lightly loaded MI355X run?  One wave per CU (or per SIMD)
 // runs a dependent v_add_f32 chain for a fixed number of instructions; wall time from HIP events, ticks from s_memtime.
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_clock.hip -o /tmp/mb_clock && /tmp/mb_clock
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define R16(x) x x x x x x x x x x x x x x x x

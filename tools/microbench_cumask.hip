@@ -1,6 +1,6 @@
 // Which physical CUs does a hipExtStreamCreateWithCUMask stream use?  For a few masks, launch 2048 one-wave
 // workgroups that record (XCC_ID, SE_ID, CU_ID) and print the set of distinct locations.
-// build: hipcc --offload-arch=gfx950 -O2 tools/microbench_cumask.hip -o tools/microbench_cumask
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/microbench_cumask.hip -o tools/microbench_cumask
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

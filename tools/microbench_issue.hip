@@ -1,6 +1,6 @@
 // tools/microbench_issue.hip -- issue cost per instruction CLASS on gfx950, in SIMD cycles per wave64 instruction: the numbers
 // behind the per-kernel "issue ms" column of profiles/r03_issue_model.txt (SQ_INSTS_VALU x class share x cost).
-//   hipcc --offload-arch=gfx950 -O3 tools/microbench_issue.hip -o /tmp/mb_issue && /tmp/mb_issue
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_issue.hip -o /tmp/mb_issue && /tmp/mb_issue
 // Every kernel is a loop of 32 independent instructions of one class (8 registers x 4), W one-wave workgroups per SIMD
 // (W = 1, 2, 4: a single wave's issue rate against the SIMD's).  The clock comes from a loop of `s_nop 15`: 16 wait states of one
 // 4-cycle issue slot each = 64 cycles (with 16 cycles the plain f32 rate would come out at 0.6 cycles per wave64 instruction, i.e.
@@ -8,7 +8,6 @@
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstring>
-typedef float v2f __attribute__((ext_vector_type(2)));
 
 #define REP4(x) x x x x
 #define KERNEL(name, TYPE, INITV, I0, I1, I2, I3, I4, I5, I6, I7) \
@@ -17,9 +16,8 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 		TYPE c = INITV; unsigned long long sm = 0; \
 		(void)c; (void)sm; \
 		for (int k = 0; k < iters; k++) { REP4(I0 I1 I2 I3 I4 I5 I6 I7) } \
-		if (iters < 0) out[threadIdx.x] = (float)(r0 + r1 + r2 + r3 + r4 + r5 + r6 + r7)SUMX + (float)sm; \
+		if (iters < 0) out[threadIdx.x] = (float)(r0 + r1 + r2 + r3 + r4 + r5 + r6 + r7) + (float)sm; \
 	}
-#define SUMX
 #define V1(op, r) asm volatile(op " %0, %0, %1" : "+v"(r) : "v"(c));
 #define VSELF(op, r) asm volatile(op : "+v"(r) : "v"(c));
 
@@ -49,13 +47,6 @@ KERNEL(k_cmp_sand, float, 1.0f, CMPBAL(r0), CMPBAL(r1), CMPBAL(r2), CMPBAL(r3), 
 KERNEL(k_salu, float, 1.0f, SXOR(r0), SXOR(r1), SXOR(r2), SXOR(r3), SXOR(r4), SXOR(r5), SXOR(r6), SXOR(r7))
 #define NOP16(r) asm volatile("s_nop 15");
 KERNEL(k_nop16, float, 1.0f, NOP16(r0), NOP16(r1), NOP16(r2), NOP16(r3), NOP16(r4), NOP16(r5), NOP16(r6), NOP16(r7))
-#undef SUMX
-#define SUMX .x
-#define PK(op, r) asm volatile(op " %0, %0, %1" : "+v"(r) : "v"(c));
-KERNEL(k_pk_add, v2f, (v2f{ 1.0f, 1.0f }), PK("v_pk_add_f32", r0), PK("v_pk_add_f32", r1), PK("v_pk_add_f32", r2), PK("v_pk_add_f32", r3), PK("v_pk_add_f32", r4), PK("v_pk_add_f32", r5), PK("v_pk_add_f32", r6), PK("v_pk_add_f32", r7))
-KERNEL(k_pk_mul, v2f, (v2f{ 1.0f, 1.0f }), PK("v_pk_mul_f32", r0), PK("v_pk_mul_f32", r1), PK("v_pk_mul_f32", r2), PK("v_pk_mul_f32", r3), PK("v_pk_mul_f32", r4), PK("v_pk_mul_f32", r5), PK("v_pk_mul_f32", r6), PK("v_pk_mul_f32", r7))
-#undef SUMX
-#define SUMX
 #define SHL64(r) asm volatile("v_lshlrev_b64 %0, 1, %0" : "+v"(r));
 KERNEL(k_shl64, unsigned long long, 77ull, SHL64(r0), SHL64(r1), SHL64(r2), SHL64(r3), SHL64(r4), SHL64(r5), SHL64(r6), SHL64(r7))
 #define FMA64(r) asm volatile("v_fma_f64 %0, %0, %1, %1" : "+v"(r) : "v"(c));
@@ -85,7 +76,7 @@ int main() {
 	const float tn = time_kernel(k_nop16, simds, iters, d);
 	const double ghz = (double)iters * 32 * 64 / (tn * 1e-3) / 1e9;
 	printf("%d CUs; clock from the s_nop loop: %.3f GHz (%.3f ms); hipDeviceProp clockRate %.3f GHz\n", prop.multiProcessorCount, ghz, tn, prop.clockRate * 1e-6);
-	const Entry es[] = { { "v_add_f32", k_add }, { "v_mul_f32", k_mul }, { "v_and_b32", k_and }, { "v_pk_add_f32", k_pk_add }, { "v_pk_mul_f32", k_pk_mul },
+	const Entry es[] = { { "v_add_f32", k_add }, { "v_mul_f32", k_mul }, { "v_and_b32", k_and },
 		{ "v_mov_b32_dpp wave_shr:1", k_mov_dpp }, { "v_add_f32_dpp wave_shr:1", k_add_dpp }, { "v_mov_b32_dpp quad_perm", k_mov_dpp_quad },
 		{ "v_bfe_i32", k_bfe }, { "v_add3_u32", k_add3 }, { "v_cndmask_b32 (vcc)", k_cndmask }, { "v_cmp_gt_f32 -> vcc", k_cmp_vcc },
 		{ "v_cmp_gt_f32 -> sgpr pair", k_cmp_sgpr }, { "v_cmp + s_and_b64 (pair)", k_cmp_sand }, { "s_xor_b64", k_salu },

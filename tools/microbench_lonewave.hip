@@ -1,7 +1,7 @@
 // tools/microbench_lonewave.hip -- what a wave that is ALONE on its SIMD pays per instruction when the instructions DEPEND on each
 // other (kv2_engine's loops are one long dependent chain): cycles per instruction for chains of several instruction kinds, and for the
 // hand-overs between the vector and the scalar unit.  One wave per CU, s_memtime around 64 x 16 instructions.
-//   hipcc --offload-arch=gfx950 -O3 tools/microbench_lonewave.hip -o /tmp/mb_lw && /tmp/mb_lw
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_lonewave.hip -o /tmp/mb_lw && /tmp/mb_lw
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define R16(x) x x x x x x x x x x x x x x x x
@@ -29,8 +29,6 @@ BENCH(k_dep_cmp_sgpr_cnd, , asm volatile("v_cmp_gt_f32_e64 %1, %0, %2\n v_cndmas
 BENCH(k_dep_readfirstlane, , asm volatile("v_readfirstlane_b32 %1, %0\n v_add_u32 %0, %1, %0" : "+v"(i), "=s"(j));)
 BENCH(k_dep_salu, , asm volatile("s_add_u32 %0, %0, 1" : "+s"(j) : : "scc");)
 BENCH(k_dep_cmp_branch, , asm volatile("v_cmp_gt_f32 vcc, %0, %1\n s_cbranch_vccz 1f\n v_add_f32 %0, %0, %1\n1:" : "+v"(a) : "v"(c) : "vcc");)
-typedef float v2f_t __attribute__((ext_vector_type(2)));
-BENCH(k_dep_pk, v2f_t p = seed;, asm volatile("v_pk_add_f32 %0, %0, %0" : "+v"(p));)
 BENCH(k_lds_rt, __shared__ int sm[64]; sm[threadIdx.x] = 0;, asm volatile("ds_read_b32 %0, %0\n s_waitcnt lgkmcnt(0)" : "+v"(i));)
 BENCH(k_mad24, , asm volatile("v_mad_u32_u24 %0, %0, %1, %1" : "+v"(i) : "v"(j));)
 BENCH(k_mul_lo, , asm volatile("v_mul_lo_u32 %0, %0, %1" : "+v"(i) : "v"(j));)
@@ -45,7 +43,7 @@ int main() {
 		{ "dependent v_xor_b32", k_dep_xor, 1 }, { "dependent v_floor_f32", k_dep_floor, 1 }, { "dependent v_bfe_i32", k_dep_bfe, 1 }, { "dependent v_bitop3_b32", k_dep_bitop3, 1 },
 		{ "dependent v_fma_f32", k_dep_fma, 1 }, { "v_cmp (vcc) -> v_cndmask, dependent", k_dep_cmp_cnd, 2 }, { "v_cmp (sgpr pair) -> v_cndmask, dependent", k_dep_cmp_sgpr_cnd, 2 },
 		{ "v_readfirstlane -> v_add (sgpr operand)", k_dep_readfirstlane, 2 }, { "dependent s_add_u32", k_dep_salu, 1 }, { "v_cmp -> s_cbranch_vccz (not taken) -> v_add", k_dep_cmp_branch, 3 },
-		{ "dependent v_pk_add_f32", k_dep_pk, 1 }, { "ds_read_b32 round trip", k_lds_rt, 1 }, { "dependent v_mad_u32_u24", k_mad24, 1 }, { "dependent v_mul_lo_u32", k_mul_lo, 1 },
+		{ "ds_read_b32 round trip", k_lds_rt, 1 }, { "dependent v_mad_u32_u24", k_mad24, 1 }, { "dependent v_mul_lo_u32", k_mul_lo, 1 },
 		{ "dependent v_lshrrev_b64", k_lshr64, 1 }, { "v_cvt_u32_f32 -> v_cvt_f32_u32", k_cvt, 2 }, { "dependent v_ffbl_b32", k_ffbl, 1 } };
 	printf("a wave alone on its SIMD (256 one-wave workgroups), cycles (s_memtime) per group of instructions, 1024 groups\n");
 	for (auto& x : e) {

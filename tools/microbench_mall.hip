@@ -6,7 +6,7 @@
 // times the read-back of C -- cold (after the caches were flushed with other data), hot (right after the write), and behind a stream
 // of A with and without the non-temporal hint.  Each read-back kernel has its own name (template tag), so a `rocprofv3 --pmc
 // FETCH_SIZE` pass of the same binary shows whether the counter moves with the timing or not.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/microbench_mall.hip -o tools/microbench_mall
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_mall.hip -o tools/microbench_mall
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,6 +1,6 @@
 // tools/microbench_rot.hip -- how fast can ONE wave run a strictly sequential complex-product recurrence
 // on gfx950?  (The CGF derotation, DSP/DSP.cpp:460-463, is 24,576 dependent steps per channel per block.)
-// Build: hipcc --offload-arch=gfx950 -O3 -ffp-contract=off tools/microbench_rot.hip -o tools/microbench_rot
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -ffp-contract=off tools/microbench_rot.hip -o tools/microbench_rot
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
@@ -8,7 +8,7 @@
 typedef float v2f __attribute__((ext_vector_type(2)));
 #define DPP_SHR1(oldv, srcv) __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(oldv), __float_as_int(srcv), 0x138, 0xF, 0xF, false))
 
-// V0: merged register (recurrence in lane 0 + history in lanes 1..63), packed math, 5 ops/step
+// V0: merged register (recurrence in lane 0 + history in lanes 1..63), 2-vector math
 __global__ __launch_bounds__(64) void v0(float2* out, float2 stp, int nchunk) {
 	v2f cur = { 1.0f, 0.0f };
 	const v2f st = { stp.x, stp.y }, sw = { -stp.y, stp.x };
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64) void v1(float2* out, float2 stp, int nchunk) {
 		out[(size_t)blockIdx.x * 64 + threadIdx.x] = make_float2(hx, hy);
 	}
 }
-// V2: scalar (unpacked) math, history apart
+// V2: scalar math, history apart
 __global__ __launch_bounds__(64) void v2(float2* out, float2 stp, int nchunk) {
 	float rx = 1.0f, ry = 0.0f, hx = 0, hy = 0;
 	for (int c = 0; c < nchunk; c++) {
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(64) void v2(float2* out, float2 stp, int nchunk) {
 		out[(size_t)blockIdx.x * 64 + threadIdx.x] = make_float2(hx, hy);
 	}
 }
-// V3: floor, packed recurrence only (no history)
+// V3: floor, 2-vector recurrence only (no history)
 __global__ __launch_bounds__(64) void v3(float2* out, float2 stp, int nchunk) {
 	v2f rot = { 1.0f, 0.0f };
 	const v2f st = { stp.x, stp.y }, sw = { -stp.y, stp.x };
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64) void v4(float2* out, float2 stp, int nchunk) {
 		out[(size_t)blockIdx.x * 64 + threadIdx.x] = make_float2(rx, ry);
 	}
 }
-// V5: history latched into LDS by lane 0 only (exec-masked ds_write), packed math
+// V5: history latched into LDS by lane 0 only (exec-masked ds_write), 2-vector math
 __global__ __launch_bounds__(64) void v5(float2* out, float2 stp, int nchunk) {
 	__shared__ float2 ring[64];
 	v2f rot = { 1.0f, 0.0f };
@@ -125,12 +125,12 @@ int main() {
 	hipMalloc(&d, 8192 * 64 * sizeof(float2));
 	const int nchunk = 24576 / 64;
 	for (int waves : { 512, 1024, 2048, 4096 }) {
-		run("v0 merged pk+dpp", v0, waves, nchunk, d);
-		run("v1 pk, dpp off chain", v1, waves, nchunk, d);
+		run("v0 merged vec+dpp", v0, waves, nchunk, d);
+		run("v1 vec, dpp off chain", v1, waves, nchunk, d);
 		run("v2 scalar, dpp off chain", v2, waves, nchunk, d);
-		run("v3 pk only (floor)", v3, waves, nchunk, d);
+		run("v3 vec only (floor)", v3, waves, nchunk, d);
 		run("v4 scalar only (floor)", v4, waves, nchunk, d);
-		run("v5 pk + lds latch lane0", v5, waves, nchunk, d);
+		run("v5 vec + lds latch lane0", v5, waves, nchunk, d);
 		run("v6 two chains per wave", v6, waves, nchunk, d);
 	}
 	return 0;

@@ -1,5 +1,5 @@
 // Issue cost of v_lshrrev_b64 against 32-bit VALU ops on gfx950 (one wave per SIMD and four waves per SIMD).
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/microbench_shift tools/microbench_shift.hip
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/microbench_shift tools/microbench_shift.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 template <int MODE>
@@ -21,11 +21,6 @@ __global__ void k(unsigned long long* out, int iters, unsigned long long seed) {
 				asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(y) : "v"(sh));
 				asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(z) : "v"(sh));
 				asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(w) : "v"(sh));
-			} else if (MODE == 2) { // packed fp32 multiply
-				asm volatile("v_pk_mul_f32 %0, %0, %0" : "+v"(a));
-				asm volatile("v_pk_mul_f32 %0, %0, %0" : "+v"(b));
-				asm volatile("v_pk_mul_f32 %0, %0, %0" : "+v"(c));
-				asm volatile("v_pk_mul_f32 %0, %0, %0" : "+v"(d));
 			} else { // v_bfe_u32
 				unsigned &x = *(unsigned*)&a, &y = *(unsigned*)&b, &z = *(unsigned*)&c, &w = *(unsigned*)&d;
 				asm volatile("v_bfe_u32 %0, %0, %1, 1" : "+v"(x) : "v"(sh));
@@ -53,6 +48,6 @@ template <int MODE> void run(const char* name, int wg) {
 	hipFree(d);
 }
 int main() {
-	for (int wg : { 256, 1024 }) { run<0>("v_lshrrev_b64", wg); run<1>("v_lshrrev_b32", wg); run<2>("v_pk_mul_f32", wg); run<3>("v_bfe_u32", wg); }
+	for (int wg : { 256, 1024 }) { run<0>("v_lshrrev_b64", wg); run<1>("v_lshrrev_b32", wg); run<2>("v_bfe_u32", wg); }
 	return 0;
 }

@@ -1,5 +1,5 @@
 // tools/microbench_stream.hip -- read-bandwidth ceilings on MI355X for the access patterns of the front end.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/microbench_stream.hip -o tools/microbench_stream
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench_stream.hip -o tools/microbench_stream
 #include <hip/hip_runtime.h>
 #include <cstdio>
 
