@@ -231,8 +231,8 @@ __device__ __forceinline__ void reg_stage(const c2 (&x)[C], HaloState<C, c2>& hs
 // pairing).  Every sum is the same pair of operands as before (float addition commutes), so the results are the same bits.
 // Lane 0's neighbour is lane 63 of the PREVIOUS tile: lane 63 leaves its five level tails of every stage in 40 bytes of LDS per
 // stage (a one-lane write), every lane reads them back at the next tile (a broadcast read; only lane 0's copy matters) and forms
-// `own + carry` with a packed addition, which the fused DPP additions then overwrite in lanes 1..63 -- no carry moves through the
-// DPP network (rounds 1-5: ten per stage and tile).  Tile loop of the four-stage ladder: 224 packed + 88 DPP -> 200 + 48 instructions.
+// `own + carry`, which the fused DPP additions then overwrite in lanes 1..63 -- no carry moves through the DPP network (without the
+// level carry: ten per stage and tile).  VALU instructions of the tile loop, four stages of CU8: 540 plain + 88 DPP -> 493 + 48.
 // Used by the integer input formats only (see k1_dpp: LC).
 // (`s_nop 1` in front of the DPP pair: a VGPR written by the preceding VALU instruction may not be read through DPP for two wait
 // states, and the compiler's hazard recogniser does not look into inline assembly.)
@@ -1821,10 +1821,10 @@ __global__ __launch_bounds__(64) void k2_cgf_search(K2Params p) {
 // window and carried across windows and blocks: a strictly sequential float recurrence of 24,576 steps
 // per (receiver, channel) and block -- no re-association is allowed, so time cannot be parallelised.
 // What CAN be done is to make the recurrence cost almost no issue slots: one LANE per chain (64
-// chains per wave), 3 packed VALU ops per step (P = (rx*sx, rx*sy), Q = (ry*-sy, ry*sx), rot' = P + Q;
+// chains per wave), six VALU operations per step (P = (rx*sx, rx*sy), Q = (ry*-sy, ry*sx), rot' = P + Q;
 // x*-y == -(x*y) exactly, so this is the reference's (ac - bd, ad + bc) bit for bit), and the phasor of
 // every step is stored time-major (rotT[n][chain]) so the 64 lanes write 512 contiguous bytes.
-// The kernel is latency bound (~20 cycles per step) but occupies only n_chan/64 waves, so it hides
+// The kernel is latency bound (~26 cycles per step) but occupies only n_chan/64 waves, so it hides
 // behind the bandwidth-bound kernels of the next block; K2c applies the phasors in parallel.
 // ------------------------------------------------------------------------------------------
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -1863,7 +1863,7 @@ __global__ __launch_bounds__(64) void k2_cgf_phasor(K2Params p) {
 }
 
 // The same recurrence without the per-sample stores: only its state at the start of every window is kept (after the
-// renormalisation).  3 packed VALU ops per step and nothing else -- in particular no store per few steps: beside the front end a
+// renormalisation).  Six VALU operations per step and nothing else -- in particular no store per few steps: beside the front end a
 // store is acknowledged after ~20 us, a wave may have 63 memory operations outstanding, and 57 checkpoints per 4.8 us window
 // stalled the recurrence at that limit (0.32 -> 0.45 ms beside the front end, the pipeline's longest chain).  The checkpoints
 // inside the windows are k2_cgf_refine's.
@@ -1898,13 +1898,12 @@ __global__ __launch_bounds__(64) void k2_cgf_phasor_ck(K2Params p) {
 }
 
 // The same once more with a chain on a PAIR of lanes (even lane: real part, odd lane: imaginary part; 32 chains per wave).
-// The packed form above takes 24 cycles per step -- three packed operations of a dependent chain, 8 cycles each; here a step
-// is own * c, partner * (-/+ s) with the partner's value through the DPP operand, and their sum: three plain operations, 4 cycles
-// each.  Every product and sum is the one of the packed form (x c + y (-s); y c + x s = x s + y c), so the states are the same bits.
-// Twice the waves: the launcher takes this form while every wave still has a SIMD of the reserved CUs to itself.  Measured alone,
-// 512 chains x 48 windows: 183 us against 247 (18 against 24 cycles per step: the DPP operand wants two wait states behind the
-// sum that wrote it, one of them an s_nop); with (own c, own s') as ONE packed product and the sum taking the partner's half through
-// DPP: 267 us -- a packed operation is 8 cycles to its dependant (profiles/r04_expC_phasor_pairs.txt).
+// The form above takes 26 cycles per step for its six operations; here a step is own * c, partner * (-/+ s) with the partner's value
+// through the DPP operand, and their sum: three operations, 4 cycles each.  Every product and sum is the one of the form above
+// (x c + y (-s); y c + x s = x s + y c), so the states are the same bits.
+// Twice the waves: the launcher takes this form while every wave still has a SIMD of the reserved CUs to itself.  24,576 steps
+// alone: 182 us against 264 (18 against 26 cycles per step: the DPP operand wants two wait states behind the sum that wrote it, one
+// of them an s_nop; profiles/plain_f32_serial_kernel_stats.txt, the recurrence of the form above in plain_f32_mb_rot.txt).
 __global__ __launch_bounds__(64) void k2_cgf_phasor_ck_pairs(K2Params p) {
 	const int lane = threadIdx.x, comp = lane & 1;
 	const int chan_raw = blockIdx.x * 32 + (lane >> 1);
@@ -2203,9 +2202,7 @@ struct PsWave {
 	unsigned long long h1, h2, h3, h4; // decisions of 1..4 symbols ago, one bit per lane
 };
 
-// M.y: the hypothesis' EMA (M.x is unused).  The step is issue-bound next to the front end, and a packed f32
-// instruction takes two issue slots on gfx950: the EMA update as one packed multiply and one packed cross add (plus the v_and for
-// |t|, which packed operands cannot take as a modifier) was five slots, the three scalar instructions below are three.
+// The step is issue-bound next to the front end: the EMA update is the three instructions below, |t| as an operand modifier.
 __device__ __forceinline__ float ps_ema(float ma, float tt) { // w * ma + (1 - w) * |t|, each product and the sum rounded (Demod.cpp:71)
 	const float w = 0.85f;
 	const float w1 = 1 - w; // (1 - weight) evaluated in float
@@ -3835,7 +3832,7 @@ __device__ __forceinline__ void v2_reset(DecReg& r) { r.state = DST_TRAINING; r.
 // as its slowest channel and every roll-back of one channel paid by ten).  What the reference computes block-wise is block-wise here,
 // with lanes over time, and only the decoders' loop is serial:
 //  * Derotate (:133-146): the phasor is rounded at every step, so every lane runs the recurrence and keeps the state in front of its
-//    own eight samples (512 steps of three packed operations -- the chain a single lane needed anyway), then derotates those eight;
+//    own eight samples (512 steps of six operations -- the chain a single lane needed anyway), then derotates those eight;
 //  * FilterFL17 (:154-167, Engine::processBlock's filter17.Run(freq_corrected, coh_filtered), :351): all 512 outputs once per block
 //    into LDS, eight per lane -- the group loop and its roll-back read them instead of filtering per decoder and sample;
 //  * the group loop: five tracker lanes + the FM decoder's lane as before; while none of the six decoders is inside a frame
